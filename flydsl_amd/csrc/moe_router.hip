@@ -348,15 +348,16 @@ __device__ __forceinline__ uint32_t keep_groups(const TopkArgs& p, int lane, int
   for (int r = 0; r < R; ++r) {
     const bool in = real && rank[r] < p.gsel;
     if (approx) {
-      // the errors of the two keys (by their sizes, which their sum may not show) and of the sum
+      // the errors of the two keys (by their sizes, which their sum may not show) and of the sum.  They differ from group
+      // to group, so a rejected group's most is held against the least of all kept ones, not of the last alone; scores
+      // that are infinite in fp32 may differ in 64 bits.
       const float fs = order_float(score[r]);
       const float close = 0.5f * (near(order_float(a[r]), p.sigmoid, pmax[r]) +
                                   (b[r] > kNone ? near(order_float(b[r]), p.sigmoid, pmax[r]) : 0.f)) +
                           0x1p-24f * __builtin_fabsf(fs);
-      const uint64_t worst = __ballot(real && rank[r] == p.gsel - 1);
-      const int last = worst ? __builtin_ctzll(worst) : 0;
-      const float edge = at_lane(fs, last) - at_lane(close, last);
-      if (__ballot(real && !in && a[r] > kNone && fs + close > edge)) unsure |= 1u << r;
+      const bool scored = real && a[r] > kNone;
+      const float edge = order_float(~wave_max(in && scored ? ~order_int(fs - close) : kNone));   // ~ turns the order round
+      if (__ballot(scored && (!(__builtin_fabsf(fs) + close < kInf) || (!in && fs + close > edge)))) unsure |= 1u << r;
     }
     if (aligned) {
 #pragma unroll

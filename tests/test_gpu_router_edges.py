@@ -1,0 +1,57 @@
+"""The router's kernels where fp32 cannot tell groups apart, against the oracle in 64 bits (oracle/router.py): ids are
+equal, and weights within the bounds of test_gpu_router.py."""
+import pytest
+import torch
+
+from test_gpu_router import check_topk, logits
+
+pytestmark = pytest.mark.gpu
+
+
+# (experts, groups): groups of whole lanes, a power of two of them, are ranked in registers, others through LDS; 8192
+# tokens up, or more than 256 experts, several rows to a wave
+@pytest.mark.parametrize("T,E,groups", [(300, 256, 8), (300, 60, 4), (8200, 256, 8), (8200, 60, 4), (8200, 6, 3), (300, 512, 16),
+                                        (300, 510, 10)])
+@pytest.mark.parametrize("size", [1e3, 2.0 ** 17])
+def test_groups_whose_two_largest_keys_cancel(gpu, T, E, groups, size):
+    """The two largest keys of every other group are +-size and leave errors of an fp32 step of that (6e-5, 2^-7) in its
+    score; the other groups' scores are exact to 1e-6.  Any of them may rank first."""
+    per = E // groups
+    x = logits(T, E, "fp32", gpu, E)
+    bias = torch.full((groups, per), -4.0 * size)
+    for g in range(groups):
+        bias[g, :2] = torch.tensor([size, -size]) if g % 2 == 0 else 0.0
+    if per > 2:                                     # not always the first two
+        bias = bias.gather(1, torch.rand(groups, per, generator=torch.Generator().manual_seed(E)).argsort(dim=1))
+    bias = bias.view(E).to(gpu)
+    for topk_groups in (1, 2, groups - 1):
+        k = 2 * topk_groups
+        for scoring in ("sigmoid", "softmax"):
+            check_topk(x, min(k, 16), scoring=scoring, bias=bias, groups=groups, topk_groups=topk_groups, grad=False)
+
+
+@pytest.mark.parametrize("T", [1, 8200])
+def test_a_group_behind_two_that_fp32_orders(gpu, T):
+    """Scores .7, .9 and .8: in fp32 the first group's keys 2^24 + .1 and .6 - 2^24 add up to 1, so that it ranks first
+    and the second, whose score is sure, last."""
+    s = torch.tensor([0.1, 0.6, 0.5, 0.4, 0.45, 0.35], dtype=torch.float64)
+    x = torch.log(s / (1 - s)).float().expand(T, 6).contiguous().to(gpu)
+    bias = torch.tensor([2.0 ** 24, -2.0 ** 24, 0, 0, 0, 0], device=gpu)
+    check_topk(x, 4, scoring="sigmoid", bias=bias, groups=3, topk_groups=2, grad=False)
+
+
+@pytest.mark.parametrize("T,E", [(40, 16), (8200, 16), (40, 12), (8200, 12), (40, 512)])
+def test_group_scores_past_the_largest_float(gpu, T, E):
+    """Sums of two keys that are infinite in fp32 and not in 64 bits, on both sides; and biases of +inf."""
+    x = logits(T, E, "fp32", gpu, 2)
+    per = E // 4
+    top = torch.tensor([2.0e38, 2.5e38, 3.0e38, 1.5e38])
+    for sign in (1.0, -1.0):
+        bias = torch.full((4, per), -3.4e38)
+        bias[:, 0], bias[:, 1] = sign * top, sign * top / 1.2
+        for topk_groups in (1, 2, 3):
+            check_topk(x, 2 * topk_groups, scoring="sigmoid", bias=bias.view(E).to(gpu), groups=4, topk_groups=topk_groups, grad=False)
+    bias = torch.zeros(4, per)
+    bias[1, 1] = bias[3, 0] = bias[3, 2] = float("inf")
+    for topk_groups in (1, 2, 3):
+        check_topk(x, 3, scoring="sigmoid", bias=bias.view(E).to(gpu), groups=4, topk_groups=topk_groups, grad=False)
