@@ -19,6 +19,7 @@ SCORING = {"softmax": 0, "sigmoid": 1}
 QUANT_MODE = {"recip_trunc": 0, "div_trunc": 1, "div_nearest": 2}
 
 MOE_SORT_MAX_EXPERTS = 512
+MOE_ROUTER_MAX_TOKENS = 2**31 - 8192
 
 # (name, restype, argtypes) for every symbol include/flygemm.h declares
 _P = ctypes.c_void_p

@@ -18,6 +18,7 @@ using namespace flygemm;
 namespace {
 
 constexpr int kMaxExperts = FLYGEMM_MOE_SORT_MAX_EXPERTS;
+constexpr int kMaxTokens = FLYGEMM_MOE_ROUTER_MAX_TOKENS;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr float kInf = __builtin_inff();
 
@@ -859,7 +860,7 @@ __device__ __forceinline__ uint32_t row_probs(const float (&x)[U][V], bool sig, 
 // 16.8 us, 4 rows 17.4; 8192 x 128 bf16 6.2 / 7.5).
 constexpr int part_rows(int V) { return V == 8 ? 4 : 8; }
 constexpr int kGradRows = 2;
-constexpr int kMaxChunk = 4096;
+constexpr int kMaxChunk = 4096;   // kMaxTokens leaves room for a chunk behind the last token, so row numbers are ints
 
 // One read of the logits; 32768 x 256 fp32 11.5 us with 16 waves to a workgroup and 8 rows of each in flight; 14.6 with
 // 4 rows one after the other, 37 with 4 waves: one wave per SIMD waits for memory.
@@ -1130,6 +1131,7 @@ void by_row(int dtype, int E, F f) {
 int check_router(const char* what, int64_t stride, int T, int E, int dtype, int scoring) {
   if (T < 0 || E < 1) return fail(hipErrorInvalidValue, "%s: invalid sizes tokens=%d experts=%d", what, T, E);
   if (E > kMaxExperts) return fail(hipErrorInvalidValue, "%s: experts=%d must be at most %d", what, E, kMaxExperts);
+  if (T > kMaxTokens) return fail(hipErrorInvalidValue, "%s: tokens=%d must be at most %d", what, T, kMaxTokens);
   if (stride < 0) return fail(hipErrorInvalidValue, "%s: negative row stride", what);
   if (dtype < FLYGEMM_QIN_F16 || dtype > FLYGEMM_QIN_F32)
     return fail(hipErrorInvalidValue, "%s: dtype %d not supported", what, dtype);
@@ -1216,7 +1218,7 @@ int flygemm_moe_topk_grad(void* dlogits, const float* dweights, const int32_t* t
 }
 
 int64_t flygemm_moe_balance_scratch(int32_t tokens, int32_t experts, int32_t sequences) {
-  if (tokens < 0 || experts < 1 || experts > kMaxExperts || sequences < 1) return -1;
+  if (tokens < 0 || tokens > kMaxTokens || experts < 1 || experts > kMaxExperts || sequences < 1) return -1;
   const int chunk = balance_chunk(tokens);
   const int64_t slots = ((int64_t)tokens + chunk - 1) / chunk + sequences, B = sequences > 1 ? sequences : 0;
   return 2 * slots * 64 * row_pack(experts) * 4 + round16(slots * 4) + round16(B * 8) + round16(B * experts * 4) + round16(B * 4);

@@ -131,8 +131,8 @@ def _check_logits(logits, scoring):
     T, E = logits.shape
     if not 0 < E <= _lib.MOE_SORT_MAX_EXPERTS:
         raise ValueError(f"{E} experts: the router's kernels take 1 to {_lib.MOE_SORT_MAX_EXPERTS}")
-    if T >= 2**31:
-        raise ValueError(f"{T} tokens do not fit 32 bits")
+    if T > _lib.MOE_ROUTER_MAX_TOKENS:
+        raise ValueError(f"{T} tokens: the router's kernels take at most {_lib.MOE_ROUTER_MAX_TOKENS}")
     if not logits.is_cuda or logits.layout is not torch.strided:
         raise ValueError(f"logits must be a dense GPU tensor, got {logits.layout} on {logits.device}")
     return T, E

@@ -292,10 +292,12 @@ int flygemm_moe_sort(int32_t* sorted_ids, float* sorted_weights, int32_t* sorted
  * (or whose key is -inf or NaN) is never chosen; a slot without an expert gets id -1 and weight 0, and so do
  * all slots of a token with token_mask[t] == 0 (bytes; NULL: none), whose logits are not read.  A NaN logit,
  * or +inf under softmax, makes the row's weights NaN.  topk at most 64, groups at most 64, experts at most
- * FLYGEMM_MOE_SORT_MAX_EXPERTS.  _grad: dlogits [tokens][experts] (contiguous, dtype) from dweights
- * [tokens][topk], with the ids of the forward call; the bias has no gradient.  No reference counterpart (its
- * harness takes torch.topk of random scores, tests/kernels/test_moe_gemm.py). */
+ * FLYGEMM_MOE_SORT_MAX_EXPERTS, tokens at most FLYGEMM_MOE_ROUTER_MAX_TOKENS (row numbers, and those that a
+ * workgroup looks ahead, fit 32 bits; the balance loss too).  _grad: dlogits [tokens][experts] (contiguous, dtype)
+ * from dweights [tokens][topk], with the ids of the forward call; the bias has no gradient.  No reference
+ * counterpart (its harness takes torch.topk of random scores, tests/kernels/test_moe_gemm.py). */
 enum { FLYGEMM_SCORE_SOFTMAX = 0, FLYGEMM_SCORE_SIGMOID = 1 };
+#define FLYGEMM_MOE_ROUTER_MAX_TOKENS (0x7fffffff - 8191)
 int flygemm_moe_topk(int32_t* topk_ids, float* topk_weights, const void* logits, int64_t row_stride, const float* bias,
                      const uint8_t* token_mask, int32_t tokens, int32_t experts, int32_t topk, int32_t groups,
                      int32_t topk_groups, int32_t dtype, int32_t scoring, int32_t renormalize, float scale,
