@@ -1236,7 +1236,8 @@ int flygemm_moe_balance(float* loss, int32_t* counts, float* aux, void* scratch,
     return fail(hipErrorInvalidValue, "%s: sequences=%d", what, sequences);
   if (tokens < 1) return fail(hipErrorInvalidValue, "%s: no tokens", what);
   const int chunk = balance_chunk(tokens);
-  if ((int64_t)chunk * topk >= (1L << 31)) return fail(hipErrorInvalidValue, "%s: topk=%d too large", what, topk);
+  // a thread's place among a chunk's ids goes up to a step behind the last
+  if ((int64_t)chunk * topk > 0x7fffffffL - kPartThreads) return fail(hipErrorInvalidValue, "%s: topk=%d too large", what, topk);
   if (!loss || !counts || !aux || !scratch || !logits || !topk_ids)
     return fail(hipErrorInvalidValue, "%s: null tensor pointer", what);
   if ((uintptr_t)scratch & 15) return fail(hipErrorInvalidValue, "%s: scratch needs 16-byte alignment", what);

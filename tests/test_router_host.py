@@ -46,3 +46,10 @@ def test_functions_refuse_too_many_tokens(call):
     x = torch.zeros(1, 8).expand(_lib.MOE_ROUTER_MAX_TOKENS + 1, 8)
     with pytest.raises(ValueError, match="tokens: the router's kernels take at most"):
         call(x)
+
+
+@pytest.mark.parametrize("tokens,k", [(1, 2**27 - 1), (1, 2**27 - 64), (25600, 21474836)])
+def test_balance_ids_of_a_chunk_do_not_fit_32_bits(tokens, k):
+    """Chunks of 16 and of 100 rows, whose ids' last place is below 2^31 and a workgroup's next one above it."""
+    assert balance(tokens, k=k) != 0
+    assert f"topk={k} too large" in _lib.load().flygemm_last_error().decode()
