@@ -325,6 +325,8 @@ def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, scoring: s
         raise TypeError("topk_ids must be an int32 or int64 tensor")
     if topk_ids.dim() != 2 or topk_ids.shape[0] != T or topk_ids.shape[1] < 1 or topk_ids.device != logits.device:
         raise ValueError(f"topk_ids must be [{T}, topk] on {logits.device}, got {tuple(topk_ids.shape)} on {topk_ids.device}")
+    if topk_ids.shape[1] >= 2**31:
+        raise ValueError(f"topk_ids has {topk_ids.shape[1]} ids a token, which do not fit 32 bits")
     cu = None
     if cu_seqlens is not None:
         cu = cu_seqlens
@@ -332,6 +334,8 @@ def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, *, scoring: s
             raise TypeError("cu_seqlens must be an int32 or int64 tensor")
         if cu.dim() != 1 or cu.numel() < 2 or cu.device != logits.device:
             raise ValueError(f"cu_seqlens must be [sequences + 1] on {logits.device}, got {tuple(cu.shape)} on {cu.device}")
+        if cu.numel() > 2**31:
+            raise ValueError(f"cu_seqlens has {cu.numel()} entries: its sequences do not fit 32 bits")
         cu = cu.to(torch.int32).contiguous()
     args = (topk_ids.contiguous(), _lib.SCORING[scoring], _check_mask(token_mask, logits), cu)
     if _differentiates(logits):

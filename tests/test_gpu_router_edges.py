@@ -3,6 +3,7 @@ equal, and weights within the bounds of test_gpu_router.py."""
 import pytest
 import torch
 
+from flydsl_amd import moe
 from test_gpu_router import check_topk, logits
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +56,14 @@ def test_group_scores_past_the_largest_float(gpu, T, E):
     bias[1, 1] = bias[3, 0] = bias[3, 2] = float("inf")
     for topk_groups in (1, 2, 3):
         check_topk(x, 3, scoring="sigmoid", bias=bias.view(E).to(gpu), groups=4, topk_groups=topk_groups, grad=False)
+
+
+def test_sizes_that_do_not_fit_32_bits_are_refused(gpu):
+    """Numbers of ids and of sequences that would reach the kernels without their upper bits (expanded tensors: nothing
+    of that size is allocated)."""
+    x = torch.zeros(1, 4, device=gpu)
+    ids = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+    with pytest.raises(ValueError, match="do not fit 32 bits"):
+        moe.moe_balance_loss(x, ids.expand(1, 2**32 + 1))
+    with pytest.raises(ValueError, match="do not fit 32 bits"):
+        moe.moe_balance_loss(x, ids, cu_seqlens=ids[0].expand(2**32 + 2))
