@@ -22,6 +22,14 @@ constexpr int kMaxTokens = FLYGEMM_MOE_ROUTER_MAX_TOKENS;
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr float kInf = __builtin_inff();
 
+// HIP launches fewer than 2^32 threads in a dimension: grids go on in y behind kGridX workgroups (of at most 1024
+// threads), and those past the last row or sequence return.
+constexpr int kGridX = 1 << 20;
+dim3 grid_of(int64_t groups) {
+  return groups <= kGridX ? dim3((unsigned)groups) : dim3(kGridX, (unsigned)((groups + kGridX - 1) / kGridX));
+}
+__device__ __forceinline__ long workgroup() { return (long)blockIdx.y * kGridX + blockIdx.x; }
+
 // ---- reductions over a wave ------------------------------------------------------------
 // one DPP step: lanes without a source keep `old`
 template <int CTRL, int ROWS>
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) moe_topk_kernel(TopkArgs p) {
   __shared__ int2 cand[kWaves][R][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long row0 = ((long)blockIdx.x * kWaves + wave) * R;
+  const long row0 = (workgroup() * kWaves + wave) * R;
   if (row0 >= p.T) return;
   constexpr bool one = R == 1;
   const int E = p.E, e0 = lane * V;
@@ -703,7 +711,7 @@ __global__ void __launch_bounds__(kThreads) moe_topk_grad_kernel(TopkGradArgs p)
   __shared__ __attribute__((aligned(32))) float lds[kWaves][R][64 * V];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long row0 = ((long)blockIdx.x * kWaves + wave) * R;
+  const long row0 = (workgroup() * kWaves + wave) * R;
   if (row0 >= p.T) return;
   constexpr bool one = R == 1;
   const int E = p.E, e0 = lane * V, at = one ? lane : lane & 15, mine = one ? 0 : lane >> 4;
@@ -953,7 +961,8 @@ __global__ void __launch_bounds__(kSumThreads) moe_balance_sum_kernel(BalArgs p)
   __shared__ __attribute__((aligned(32))) double lp[kSumWaves / 2][64 * V];
   __shared__ __attribute__((aligned(32))) int lc[kSumWaves / 2][64 * V];
   __shared__ int ln;
-  const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.x, E = p.E, e0 = lane * V;
+  if (workgroup() >= p.B) return;
+  const int tid = threadIdx.x, lane = tid & 63, b = (int)workgroup(), E = p.E, e0 = lane * V;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo = p.cu ? seq_begin(p.cu, b, p.T) : 0, hi = p.cu ? seq_begin(p.cu, b + 1, p.T) : p.T;
   const int c0 = lo / p.chunk, c1 = lo < hi ? (hi - 1) / p.chunk + 1 : c0;
@@ -1059,7 +1068,7 @@ __global__ void __launch_bounds__(kThreads) moe_balance_grad_kernel(BalGradArgs 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int E = p.E, e0 = lane * V;
-  const long first = ((long)blockIdx.x * kWaves + wave) * kGradRows;
+  const long first = (workgroup() * kWaves + wave) * kGradRows;
   if (first >= p.T) return;
   const float scale = *p.dloss * p.aux[(int64_t)p.B * E];
   int b = p.cu ? seq_of(p.cu, p.B, (int)first) : 0;
@@ -1178,7 +1187,7 @@ int flygemm_moe_topk(int32_t* topk_ids, float* topk_weights, const void* logits,
              packs_fit(logits, row_stride, experts, dtype), scale};
   const bool many = several_rows(tokens, experts, topk);
   const long per_wg = (long)kWaves * (many ? choice_rows(row_pack(experts)) : 1);
-  const dim3 grid((unsigned)((tokens + per_wg - 1) / per_wg));
+  const dim3 grid = grid_of((tokens + per_wg - 1) / per_wg);
   by_row(dtype, experts, [&](auto t, auto v) {
     typedef decltype(t) T;
     constexpr int V = decltype(v)::value;
@@ -1206,7 +1215,7 @@ int flygemm_moe_topk_grad(void* dlogits, const float* dweights, const int32_t* t
                  scale};
   const bool many = several_rows(tokens, experts, topk);
   const long per_wg = (long)kWaves * (many ? choice_rows(row_pack(experts)) : 1);
-  const dim3 grid((unsigned)((tokens + per_wg - 1) / per_wg));
+  const dim3 grid = grid_of((tokens + per_wg - 1) / per_wg);
   by_row(dtype, experts, [&](auto t, auto v) {
     typedef decltype(t) T;
     constexpr int V = decltype(v)::value;
@@ -1268,7 +1277,7 @@ int flygemm_moe_balance(float* loss, int32_t* counts, float* aux, void* scratch,
   });
   if ((rc = launched(what))) return rc;
   by_row(FLYGEMM_QIN_F32, experts, [&](auto, auto v) {
-    hipLaunchKernelGGL((moe_balance_sum_kernel<decltype(v)::value>), dim3((unsigned)sequences), dim3(kSumThreads), 0, st, a);
+    hipLaunchKernelGGL((moe_balance_sum_kernel<decltype(v)::value>), grid_of(sequences), dim3(kSumThreads), 0, st, a);
   });
   if ((rc = launched(what))) return rc;
   if (sequences > 1) {
@@ -1291,7 +1300,7 @@ int flygemm_moe_balance_grad(void* dlogits, const float* dloss, const float* aux
   BalGradArgs a{dlogits, dloss, aux, logits, token_mask, cu_seqlens, row_stride, tokens, experts, sequences,
                 scoring == FLYGEMM_SCORE_SIGMOID, packs_fit(logits, row_stride, experts, dtype),
                 packs_fit(dlogits, experts, experts, dtype)};
-  const dim3 grid((unsigned)(((long)tokens + kWaves * kGradRows - 1) / (kWaves * kGradRows)));
+  const dim3 grid = grid_of(((int64_t)tokens + kWaves * kGradRows - 1) / (kWaves * kGradRows));
   by_row(dtype, experts, [&](auto t, auto v) {
     hipLaunchKernelGGL((moe_balance_grad_kernel<decltype(t), decltype(v)::value>), grid, dim3(kThreads), 0,
                        (hipStream_t)stream, a);

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from flydsl_amd import moe
-from test_gpu_router import check_topk, logits
+from test_gpu_router import U, check_topk, logits, np64, within
+from oracle import router as orr
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,63 @@ def test_sizes_that_do_not_fit_32_bits_are_refused(gpu):
         moe.moe_balance_loss(x, ids.expand(1, 2**32 + 1))
     with pytest.raises(ValueError, match="do not fit 32 bits"):
         moe.moe_balance_loss(x, ids, cu_seqlens=ids[0].expand(2**32 + 2))
+
+
+def same_rows(t):
+    """Whether all rows are equal, without a copy of the whole."""
+    return all(bool((part == t[:1]).all()) for part in t.split(1 << 24))
+
+
+@pytest.mark.parametrize("T,E,k", [(2**26 + 5, 17, 17), (2**28 + 7, 2, 1)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_topk_of_more_workgroups_than_one_dimension_takes(gpu, T, E, k, with_bias):
+    """2^32 threads and more, one row to a wave and four: every row of a broadcast one gives what that row gives."""
+    x = torch.randn(1, E, generator=torch.Generator().manual_seed(E)).to(gpu)
+    bias = torch.zeros(E, device=gpu) if with_bias else None
+    leaf = x.expand(T, E).requires_grad_()
+    ids, w = moe.moe_topk(leaf, k, scoring="softmax", correction_bias=bias, renormalize=False)
+    rid, rw = orr.topk(np64(x), k, "softmax", None, 1, 1, False)
+    assert ids[0].tolist() == rid[0].tolist() and same_rows(ids)
+    # 2 R + 32 steps of 2^-23, as in test_gpu_router.py, with R < 8
+    within(w[:1], rw, 48 * U * rw, "weights")
+    assert same_rows(w.detach())
+    dw = torch.randn(1, k, generator=torch.Generator().manual_seed(1)).to(gpu)
+    (dx,) = torch.autograd.grad(w, leaf, dw.expand(T, k))
+    ref = orr.topk_grad(np64(x), rid, np64(dw), "softmax", False)
+    within(dx[:1], ref, 64 * U * orr.scores(np64(x)[0], "softmax") * (abs(np64(dw[0, :]))[None].max() * 2) + 1e-37, "gradient")
+    assert same_rows(dx)
+
+
+def test_balance_gradient_of_more_workgroups_than_one_dimension_takes(gpu):
+    """2^28 tokens of one row of logits, all of them with expert 0: f = (2, 0), P = p, and every row's gradient
+    p (f - f.p) / T."""
+    T = 2**28 + 7
+    x = torch.tensor([[0.3, -0.4]], device=gpu)
+    leaf = x.expand(T, 2).requires_grad_()
+    loss, counts = moe.moe_balance_loss(leaf, torch.zeros(1, 1, dtype=torch.int32, device=gpu).expand(T, 1))
+    p = torch.softmax(x.double(), dim=1)[0].cpu()
+    assert counts.tolist() == [T, 0]
+    assert abs(loss.item() - 2 * p[0].item()) <= (2 + 32 + 4096) * U * 2 * p[0].item()
+    (dx,) = torch.autograd.grad(loss, leaf)
+    h = torch.tensor([2.0, 0.0], dtype=torch.float64) / T
+    want = p * (h - (p * h).sum())
+    assert ((dx[0].cpu() - want).abs() <= 50 * U * p * 2 * h.max()).all()
+    assert same_rows(dx)
+
+
+def test_balance_of_more_sequences_than_one_dimension_takes(gpu):
+    """2^22 sequences, most of them empty, of one token each otherwise: L_b = E p[id] and f = E at the token's expert."""
+    T, E, B = 1000, 3, 2**22 + 11
+    x = logits(T, E, "fp32", gpu, 1)
+    ids = torch.arange(T, device=gpu).remainder(E).to(torch.int32)[:, None]
+    cu = (torch.arange(B + 1, device=gpu) * T // B).to(torch.int32)
+    leaf = x.clone().requires_grad_()
+    loss, counts = moe.moe_balance_loss(leaf, ids, cu_seqlens=cu)
+    p = torch.softmax(x.double(), dim=1)
+    want = E * p.gather(1, ids.long()).mean()
+    assert counts.tolist() == [334, 333, 333]
+    assert abs(loss.item() - want.item()) <= (2 * 12 + 33) * U * want.item()
+    (dx,) = torch.autograd.grad(loss, leaf)
+    h = torch.zeros_like(p).scatter_(1, ids.long(), E / T)
+    want = p * (h - (p * h).sum(dim=1, keepdim=True))
+    assert ((dx - want).abs() <= (2 * 12 + 48) * U * p * 2 * E / T + 1e-37).all()
