@@ -118,12 +118,13 @@ class BlockscaleGemmEpilogue:
         _lib.check(rc, "flygemm_blockscale_epilogue")
 
     def _bind(self):
-        """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``)."""
+        """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``), and
+        the bias's and residual's types: the bias's chooses how it is read."""
         g, act = self.gemm, self._act
         fn = _lib.load().flygemm_blockscale_epilogue
         K, sbk, out, var = g.K, g.scale_block_k, _lib.FLYGEMM_OUT[g.out_dtype], g.variant
         sk = K // sbk
-        check, f32, code32 = _lib.check, torch.float32, _lib.FLYGEMM_OUT["fp32"]
+        check, f32, out_t, code32 = _lib.check, torch.float32, _OUT_TORCH[g.out_dtype], _lib.FLYGEMM_OUT["fp32"]
 
         def call(c, a, b, sa, sb, bias, res, M, N, stream=None):
             s = 0 if stream is None else (stream if type(stream) is int else stream.cuda_stream)
@@ -131,6 +132,10 @@ class BlockscaleGemmEpilogue:
                     or sb.numel() < (N + 127) // 128 * sk or (bias is not None and bias.numel() < N)
                     or (res is not None and res.numel() < M * N)):
                 raise ValueError(f"a tensor is too small for M={M}, N={N}, K={K}")
+            if ((bias is not None and bias.dtype is not f32 and bias.dtype is not out_t)
+                    or (res is not None and res.dtype is not out_t)):
+                raise TypeError(f"bias is fp32 or {out_t}, residual {out_t}: got {bias if bias is None else bias.dtype} "
+                                f"and {res if res is None else res.dtype}")
             rc = fn(c.data_ptr(), a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(),
                     None if bias is None else bias.data_ptr(), None if res is None else res.data_ptr(), M, N, K, sbk, out,
                     code32 if bias is None or bias.dtype is f32 else out, act, var, s)

@@ -265,11 +265,12 @@ class PreshuffleGemmEpilogue:
         _lib.check(rc, "flygemm_mxfp4_epilogue" if fp4 else "flygemm_preshuffle_epilogue")
 
     def _bind(self):
-        """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``)."""
+        """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``), and
+        the bias's and residual's types: the bias's chooses how it is read."""
         g, act = self.gemm, self._act
         lib = _lib.load()
         K, var, out = g.K, g.variant, _lib.FLYGEMM_OUT[g.out_dtype]
-        check, f32, code32 = _lib.check, torch.float32, _lib.FLYGEMM_OUT["fp32"]
+        check, f32, out_t, code32 = _lib.check, torch.float32, _OUT_TORCH[g.out_dtype], _lib.FLYGEMM_OUT["fp32"]
         fp4 = g.in_dtype == "fp4"
         scaled = g.in_dtype not in _IN_TORCH16
         fn = lib.flygemm_mxfp4_epilogue if fp4 else lib.flygemm_preshuffle_epilogue
@@ -285,6 +286,10 @@ class PreshuffleGemmEpilogue:
                     or (scaled and (sa.numel() < ((M + 31) // 32 * 32 if fp4 else M) * ks or sb.numel() < N * ks))
                     or (bias is not None and bias.numel() < N) or (res is not None and res.numel() < M * N)):
                 raise ValueError(f"a tensor is too small for M={M}, N={N}, K={K}")
+            if ((bias is not None and bias.dtype is not f32 and bias.dtype is not out_t)
+                    or (res is not None and res.dtype is not out_t)):
+                raise TypeError(f"bias is fp32 or {out_t}, residual {out_t}: got {bias if bias is None else bias.dtype} "
+                                f"and {res if res is None else res.dtype}")
             rc = fn(c.data_ptr(), a.data_ptr(), b.data_ptr(), sa.data_ptr() if scaled else None,
                     sb.data_ptr() if scaled else None, None if bias is None else bias.data_ptr(),
                     None if res is None else res.data_ptr(), M, N, K, *kinds,

@@ -56,3 +56,27 @@ def test_builders_refuse():
         launch(t, t, t, t, t, None, None, M, N)
     with pytest.raises(TypeError, match="stream"):
         launch(t, t, t, t, t, None, None, M, N, "stream")
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8_block", "fp4"])
+@pytest.mark.parametrize("out", ["bf16", "fp16"])
+def test_bound_calls_refuse_types(kind, out):
+    """flydsl_amd.compile's call: a bias that is neither fp32 nor the output's type would be read as the output's, and one of
+    one-byte elements, or such a residual, past its end."""
+    m, n, k = 4, 64, 256
+    if kind == "fp8_block":
+        launch = compile_blockscale_preshuffle_gemm_epilogue(K=k, out_dtype=out)
+    else:
+        launch = compile_preshuffle_gemm_epilogue(K=k, tile_m=64, tile_n=64, tile_k=256, in_dtype=kind, out_dtype=out)
+    call = launch._bind()
+    ot, other = (torch.bfloat16, torch.float16) if out == "bf16" else (torch.float16, torch.bfloat16)
+    codes, scales = torch.zeros(n * k, dtype=torch.int8), torch.ones(32 * k)
+    c, bias, res = torch.zeros(m, n, dtype=ot), torch.zeros(n), torch.zeros(m, n, dtype=ot)
+    for t in (torch.float64, other, torch.int8, torch.int32):
+        with pytest.raises(TypeError, match="bias is fp32 or"):
+            call(c, codes, codes, scales, scales, bias.to(t), res, m, n)
+    for t in (torch.float32, other, torch.uint8):
+        with pytest.raises(TypeError, match="residual"):
+            call(c, codes, codes, scales, scales, None, res.to(t), m, n)
+        with pytest.raises(TypeError, match="residual"):
+            call(c, codes, codes, scales, scales, bias.to(ot), res.to(t), m, n)
