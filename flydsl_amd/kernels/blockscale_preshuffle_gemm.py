@@ -119,7 +119,8 @@ class BlockscaleGemmEpilogue:
 
     def _bind(self):
         """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``), and
-        the bias's and residual's types: the bias's chooses how it is read."""
+        the bias's and residual's types (the bias's chooses how it is read) and layouts (an expanded one has more
+        elements than memory)."""
         g, act = self.gemm, self._act
         fn = _lib.load().flygemm_blockscale_epilogue
         K, sbk, out, var = g.K, g.scale_block_k, _lib.FLYGEMM_OUT[g.out_dtype], g.variant
@@ -136,6 +137,8 @@ class BlockscaleGemmEpilogue:
                     or (res is not None and res.dtype is not out_t)):
                 raise TypeError(f"bias is fp32 or {out_t}, residual {out_t}: got {bias if bias is None else bias.dtype} "
                                 f"and {res if res is None else res.dtype}")
+            if (bias is not None and not bias.is_contiguous()) or (res is not None and not res.is_contiguous()):
+                raise ValueError("bias and residual must be contiguous")
             rc = fn(c.data_ptr(), a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(),
                     None if bias is None else bias.data_ptr(), None if res is None else res.data_ptr(), M, N, K, sbk, out,
                     code32 if bias is None or bias.dtype is f32 else out, act, var, s)

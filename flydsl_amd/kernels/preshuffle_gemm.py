@@ -266,7 +266,8 @@ class PreshuffleGemmEpilogue:
 
     def _bind(self):
         """The launch with only its bounds checks, for ``flydsl_amd.compile`` (as ``PreshuffleGemm._bind``), and
-        the bias's and residual's types: the bias's chooses how it is read."""
+        the bias's and residual's types (the bias's chooses how it is read) and layouts (an expanded one has more
+        elements than memory)."""
         g, act = self.gemm, self._act
         lib = _lib.load()
         K, var, out = g.K, g.variant, _lib.FLYGEMM_OUT[g.out_dtype]
@@ -290,6 +291,8 @@ class PreshuffleGemmEpilogue:
                     or (res is not None and res.dtype is not out_t)):
                 raise TypeError(f"bias is fp32 or {out_t}, residual {out_t}: got {bias if bias is None else bias.dtype} "
                                 f"and {res if res is None else res.dtype}")
+            if (bias is not None and not bias.is_contiguous()) or (res is not None and not res.is_contiguous()):
+                raise ValueError("bias and residual must be contiguous")
             rc = fn(c.data_ptr(), a.data_ptr(), b.data_ptr(), sa.data_ptr() if scaled else None,
                     sb.data_ptr() if scaled else None, None if bias is None else bias.data_ptr(),
                     None if res is None else res.data_ptr(), M, N, K, *kinds,

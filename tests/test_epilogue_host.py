@@ -80,3 +80,21 @@ def test_bound_calls_refuse_types(kind, out):
             call(c, codes, codes, scales, scales, None, res.to(t), m, n)
         with pytest.raises(TypeError, match="residual"):
             call(c, codes, codes, scales, scales, bias.to(ot), res.to(t), m, n)
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8_block"])
+def test_bound_calls_refuse_layouts(kind):
+    """An expanded bias or residual has as many elements as the call needs, but not as much memory."""
+    m, n, k = 4, 64, 256
+    if kind == "fp8_block":
+        launch = compile_blockscale_preshuffle_gemm_epilogue(K=k, out_dtype="bf16")
+    else:
+        launch = compile_preshuffle_gemm_epilogue(K=k, tile_m=64, tile_n=64, tile_k=256, in_dtype=kind, out_dtype="bf16")
+    call = launch._bind()
+    codes, scales = torch.zeros(n * k, dtype=torch.int8), torch.ones(n * k)
+    c = torch.zeros(m, n, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="contiguous"):
+        call(c, codes, codes, scales, scales, torch.zeros(1).expand(n), c, m, n)
+    for res in (c[:1].expand(m, n), torch.zeros(n, m, dtype=torch.bfloat16).t()):
+        with pytest.raises(ValueError, match="contiguous"):
+            call(c, codes, codes, scales, scales, None, res, m, n)
