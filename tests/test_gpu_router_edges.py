@@ -1,5 +1,6 @@
-"""The router's kernels where fp32 cannot tell groups apart, against the oracle in 64 bits (oracle/router.py): ids are
-equal, and weights within the bounds of test_gpu_router.py."""
+"""The router's kernels where fp32 cannot tell groups apart, on special values with several rows to a wave, and at sizes
+near their limits, against the oracle in 64 bits (oracle/router.py): ids are equal, and weights within the bounds of
+test_gpu_router.py."""
 import pytest
 import torch
 
@@ -128,3 +129,46 @@ def test_balance_of_more_sequences_than_one_dimension_takes(gpu):
     h = torch.zeros_like(p).scatter_(1, ids.long(), E / T)
     want = p * (h - (p * h).sum(dim=1, keepdim=True))
     assert ((dx - want).abs() <= (2 * 12 + 48) * U * p * 2 * E / T + 1e-37).all()
+
+
+def special_rows(T, E, dev):
+    """Rows of infinities, NaN and the type's lowest value, ordinary ones between and behind them; a mask."""
+    inf, nan = float("inf"), float("nan")
+    x = logits(T, E, "fp32", dev, 3)
+    low = torch.finfo(torch.float32).min
+    x[0] = -inf
+    x[1, 3:] = -inf
+    x[2, 0] = -inf
+    x[3] = low
+    x[5, 5:] = low
+    x[6, 7] = nan
+    x[7] = nan
+    x[9, 9] = inf
+    x[10] = inf
+    x[11, ::2], x[11, 1::2] = inf, -inf
+    x[12, 0], x[12, 1], x[12, 2] = nan, inf, -inf
+    x[13] *= 1e4
+    x[14] -= 500.0                     # sigmoid underflows in fp32
+    x[15] += 500.0
+    x[17, 3] = -low
+    x[18] = -low
+    x[19:22] = nan                     # masked
+    x[22] = inf
+    x[-1, E - 1] = nan                 # of the last wave, which may have rows to spare
+    mask = torch.ones(T, dtype=torch.bool, device=dev)
+    mask[19:23] = False
+    return x, mask
+
+
+@pytest.mark.parametrize("T,E,k", [(8201, 40, 6), (8201, 40, 16), (8203, 60, 4), (101, 512, 8), (102, 300, 16)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_special_values_with_several_rows_to_a_wave(gpu, T, E, k, scoring):
+    x, mask = special_rows(T, E, gpu)
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(2)).mul_(0.1).to(gpu)
+    special = bias.clone()
+    special[4], special[9], special[11] = float("-inf"), float("nan"), float("inf")
+    tied = torch.zeros_like(bias)
+    for b in (None, bias, special, tied):
+        for g, tg in ((1, 1), (5 if E % 5 == 0 else 4, 3)):
+            if k <= E // g * tg:
+                check_topk(x, k, scoring=scoring, bias=b, groups=g, topk_groups=tg, renorm=b is not bias, mask=mask, grad=b is bias)
