@@ -233,18 +233,16 @@ def _linear_plan(s):
 
     c = s["case"]
     M, N, K, kind, dev = c["M"], c["N"], c["K"], c["kind"], s["a"].device
-    sa, sb = s["sa"], s["sb"]
+    sb = s["sb"]
     if kind == "mxfp4":
-        a, b = fp4.pack_fp4(s["a"])[:M].contiguous(), fp4.shuffle_weight_w4(fp4.pack_fp4(s["b"]))
-        sa, sb = fp4.shuffle_scale_w4(sa), fp4.shuffle_scale_w4(sb)
+        s["fp4"] = fp4
+        b, sb = fp4.shuffle_weight_w4(fp4.pack_fp4(s["b"])), fp4.shuffle_scale_w4(sb)
     else:
-        a, b = s["a"], fly.shuffle_weight(s["b"])
+        b = fly.shuffle_weight(s["b"])
         if kind == "int4":
             b = fly.pack_int4(b)
-        elif kind == "fp8_block":
-            sa = sa.t().contiguous()
-    if sa is None:
-        sa = sb = torch.empty(0, dtype=torch.float32, device=dev)
+    if s["sa"] is None:
+        s["sa"] = sb = torch.empty(0, dtype=torch.float32, device=dev)
     kw = dict(M=M, N=N, K=K, tile_m=64, tile_n=64, out_dtype=c["out"], activation=c["act"])
     if kind == "fp8_block":
         launch = compile_blockscale_preshuffle_gemm_epilogue(tile_k=128, **kw)
@@ -252,11 +250,20 @@ def _linear_plan(s):
         tile_k = {"mxfp4": 256, "fp8": 128, "bf16": 32, "fp16": 32}.get(kind, 64)
         launch = compile_preshuffle_gemm_epilogue(tile_k=tile_k, in_dtype="fp4" if kind == "mxfp4" else kind, **kw)
     out = torch.empty(M, N, dtype=T16[c["out"]], device=dev)
-    flat = [t.view(-1) for t in (out, a, b, sa, sb)]
-    for k in ("a", "b", "sa", "sb"):
-        del s[k]
-    s.update(out=out, args=(*flat, s["bias"], s["res"], M, N))
-    s["launch"] = fly.compile(launch, *s["args"], torch.cuda.current_stream())
+    s.update(out=out, args=(out, s["a"], b, s["sa"], sb, s["bias"], s["res"], M, N))
+    s["launch"] = fly.compile(launch, *_linear_args(s), torch.cuda.current_stream())
+
+
+def _linear_args(s):
+    """The launcher's arguments, the activations laid out as it takes them: MXFP4 codes two to a byte and their scales in
+    tiles, block scales K-block major."""
+    kind = s["case"]["kind"]
+    if kind not in ("mxfp4", "fp8_block"):
+        return s["args"]
+    out, a, b, sa, *rest = s["args"]
+    if kind == "mxfp4":
+        return out, s["fp4"].pack_fp4(a)[:rest[-2]], b, s["fp4"].shuffle_scale_w4(sa), *rest
+    return out, a, b, sa.t().contiguous(), *rest
 
 
 # ---- one pass ------------------------------------------------------------------------------
@@ -267,7 +274,7 @@ def run(state):
 def _run_own(s):
     c = s["case"]
     if c["op"] == "linear":
-        s["launch"](*s["args"], torch.cuda.current_stream())
+        s["launch"](*_linear_args(s), torch.cuda.current_stream())
         return s["out"]
     moe = s["moe"]
     if c["op"] == "topk":
