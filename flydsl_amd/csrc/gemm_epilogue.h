@@ -8,9 +8,11 @@
 //              negative x, and x^2 past the largest float still gives x or 0
 //   gelu       0.5 x erfc(-x / sqrt 2).  For z >= 0 erfc(z) / 2 = t P(t) exp(-z^2) with t = 1 / (1 + 0.46 z):
 //              erfcx(z) / t is smooth over t in (0, 1], and P its polynomial of degree 7, fitted in the relative error
-//              (7e-7).  With h = erfc(|x| / sqrt 2) / 2, x < 0 takes x h and x >= 0 x (1 - h), so neither side cancels.
-//              In fp32 within 2.2e-6 of the value for |x| < 6 and 8e-6 to |x| = 14 (the exponent's rounding),
-//              against 2.4e-4, half a step of an fp16 output.
+//              (7e-7; degree 8 reaches 1.3e-7 for one more instruction a value, behind which exp2's argument and the
+//              reciprocal leave 1e-6 all the same).  With h = erfc(|x| / sqrt 2) / 2, x < 0 takes x h and x >= 0
+//              x (1 - h), so neither side cancels.  In fp32 within 2.2e-6 of the value for |x| < 6 and 9e-6 to
+//              |x| = 13 (the exponent's rounding), against 2.4e-4, half a step of an fp16 output.  From x = -13.05 the
+//              value is below the smallest normal number, and from -13.2 exp2 gives 0 for it (5e-39 off at most).
 // Which activation is a wave-uniform branch on a kernel argument, around all of a tile's values (or half of
 // them): five kernels in its place would be five times the library.  Branching per four values inside the
 // unrolled code cost more than most activations: the path taken hopped through 60 KB of instructions.

@@ -151,9 +151,12 @@ __device__ __forceinline__ void store_row(T* row, int E, int lane, bool vec, con
   }
 }
 
-// exp of a difference to a row's maximum: the hardware's exp2, whose argument is rounded by 2^-24 of itself
+// exp of a difference to a row's maximum: the hardware's exp2 (1 ulp), whose argument is rounded by 2^-24 of itself.  For
+// sums of a row and terms next to them, where that is R 2^-24 of the value, R the row's range (expf keeps its argument
+// exact, for several instructions more); weights that are returned take expf.
 __device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
-// expf rather than exp_fast: for x far below 0 the relative error of the result is that of exp(-x)
+// expf rather than exp_fast: for x far below 0 the relative error of the result is that of exp(-x).  The hardware's
+// reciprocal is within 1 ulp; a division, within half of one, takes several instructions more.
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + expf(-x)); }
 __device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
 
@@ -177,6 +180,8 @@ constexpr int choice_rows(int V) { return V == 8 ? 2 : 4; }
 // MI355X, top-8 sigmoid, one row / several: 2048 x 256 4.2 us / 5.9, 4096 x 256 5.4 / 6.1, 8192 x 256 7.6 / 6.9, 16384 x 256
 // 12.4 / 9.0, 8192 x 128 5.7 / 5.8, 16384 x 64 7.5 / 6.8); with more than 256 experts always, whose lists of eight choose_row sorts
 // in every lane (2048 x 512 8.8 / 5.7, 16384 x 512 45.3 / 12.6).  The gradients differ by less (16384 x 256 6.9 / 6.1).
+// Above 16 ids there is one row to a wave, and its time grows with k (softmax without a bias, k = 16 / 17 / 32 / 64:
+// 32768 x 256 22.5 / 36 / 57 / 102, 16384 x 512 18 / 67 / 104 / 182).
 constexpr int kManyTokens = 8192;
 bool several_rows(int tokens, int experts, int topk) {
   return topk <= 16 && (experts > 256 || tokens >= kManyTokens);
@@ -216,9 +221,10 @@ __device__ __forceinline__ float chosen_score(bool one, bool sig, bool renorm, b
 // Two fp32 keys closer than this may be in the other order in 64 bits: twice a key's error.  u = 2^-24:
 //   sigmoid  exp2 2 u and its argument 1.22 |x| u, both of e = exp(-x), count s (1 - s) <= 0.25 and s (1 - s) |x| <= 0.23
 //            times; 1 + e and the reciprocal u each (s < 1): 2.8 u in all
-//   softmax  of p: the same two errors of its own exp2 (p |x - m| <= 0.37), and the sum's: the terms' arguments
-//            1.22 ln 512 u on average, 14 additions, exp2, reciprocal and product: 30 u p + 0.5 u
-// and the sum with the bias u |key|.
+//   softmax  of p: the same two errors of its own exp2 and the difference's u |x - m| (p |x - m| <= 0.37), and the sum's:
+//            the terms' differences and arguments 2.22 ln 512 u on average, 14 additions, exp2, reciprocal and product:
+//            33 u p + 0.9 u in all
+// and the sum with the bias u |key|.  Taken are 4 u, 40 u pmax + 2 u, and 2 u |key|.
 __device__ __forceinline__ float near(float key, bool sig, float pmax) {
   return sig ? 0x1p-21f + 0x1p-22f * __builtin_fabsf(key)
              : 0x1.4p-18f * pmax + 0x1p-22f * (1.f + __builtin_fabsf(key));
@@ -423,7 +429,8 @@ __device__ __forceinline__ int choose_row(int k, int lane, int first, const int 
 // is found by counting (downwards from the largest key in growing steps, then by halves); the keys that
 // reach it go to the row's 16 lanes in order of their experts, through LDS, and there every lane counts the
 // larger ones, which is its place.  Against taking the largest k times (choose_row, whose lists are popped in every
-// lane for each), 471 -> 289 vector instructions a row of 256 experts with groups and a bias.  A row with more than 16 keys
+// lane for each), the whole kernel took 289 vector instructions a row of 256 experts with groups and a bias in place of
+// 471; what settles doubts in 64 bits has made them 327.  A row with more than 16 keys
 // that tie at its threshold takes choose_row.  The lanes behind the k-th hold the next candidates; their number is
 // returned (of the lane's row), and rest is at least the largest key that is no candidate.
 template <int V, int R>
@@ -529,8 +536,9 @@ __device__ __forceinline__ void order64(int lane, double key, int& id) {
 // fp32, such sums tie or swap for logits that differ, so where fp32 keys come closer than their errors, keys in 64
 // bits decide: among a row's candidates, or, where the candidates or the groups are in doubt, the row again.  Without a bias the keys are
 // the logits, and exact.
-// Bound by issue: 32768 x 256 rows with groups and a bias 23.6 us (25.6 with every row in doubt chosen again, of which ten
-// made the whole launch wait), all of it in 64 bits one row at a time 68; 13.4 without a bias.
+// Bound by issue: 32768 x 256 rows with groups and a bias 25 us (0.4 of it the bounds of every kept group; 2 more with
+// every row in doubt chosen again, of which ten made the whole launch wait), all of it in 64 bits one row at a time 68;
+// 13.5 without a bias.
 template <typename T, int V, bool BIAS, int R>
 __global__ void __launch_bounds__(kThreads) moe_topk_kernel(TopkArgs p) {
   __shared__ double lds[kWaves][64 * V];
@@ -705,7 +713,7 @@ struct TopkGradArgs {
 // dx_i = t_i (softmax) or t_i sigmoid(-x_i) for the chosen, and without renorm the softmax's
 // -p_e sum t for every expert.  R rows to a wave as in the choice, row r's ids in lanes 16 r to 16 r + 15; their
 // values go to the rows' experts through LDS.  Bound by writing [T][E]: 32768 x 256 fp32 9.0 us, one row to a wave and its
-// ids handed round one by one 18.6.
+// ids handed round one by one 18.6.  A dense gradient (softmax without renorm) takes exp_fast for p, as the row's sum.
 template <typename T, int V, int R>
 __global__ void __launch_bounds__(kThreads) moe_topk_grad_kernel(TopkGradArgs p) {
   __shared__ __attribute__((aligned(32))) float lds[kWaves][R][64 * V];
@@ -870,7 +878,10 @@ constexpr int part_rows(int V) { return V == 8 ? 4 : 8; }
 constexpr int kGradRows = 2;
 constexpr int kMaxChunk = 4096;   // kMaxTokens leaves room for a chunk behind the last token, so row numbers are ints
 
-// One read of the logits; 32768 x 256 fp32 11.5 us with 16 waves to a workgroup and 8 rows of each in flight; 14.6 with
+// A lane adds its experts' probabilities over the rows of its wave in fp32, the waves' sums in fp32 too: at most 4096 / 16
+// additions of terms that are all positive, 2^-16 of the sum at worst and 6e-8 of the loss as measured, for half the registers of 64 bits;
+// the chunks' sums are added in 64 bits (moe_balance_sum_kernel).
+// One read of the logits; 32768 x 256 fp32 11.5-12 us with 16 waves to a workgroup and 8 rows of each in flight; 14.6 with
 // 4 rows one after the other, 37 with 4 waves: one wave per SIMD waits for memory.
 constexpr int kPartThreads = 1024, kPartWaves = kPartThreads / 64;
 template <typename T, int V>
