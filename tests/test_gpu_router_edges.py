@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from flydsl_amd import moe
-from test_gpu_router import U, check_topk, logits, np64, within
+from test_gpu_router import DT, U, check_topk, logits, np64, within
 from oracle import router as orr
 
 pytestmark = pytest.mark.gpu
@@ -172,3 +172,17 @@ def test_special_values_with_several_rows_to_a_wave(gpu, T, E, k, scoring):
         for g, tg in ((1, 1), (5 if E % 5 == 0 else 4, 3)):
             if k <= E // g * tg:
                 check_topk(x, k, scoring=scoring, bias=b, groups=g, topk_groups=tg, renorm=b is not bias, mask=mask, grad=b is bias)
+
+
+@pytest.mark.parametrize("T", [40, 8200])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_subnormal_logits_are_ordered(gpu, T, dtype):
+    """Logits that are all below the type's smallest normal number, of both signs, and zeros of both signs among them."""
+    fin = torch.finfo(DT[dtype])
+    step = fin.smallest_normal * fin.eps
+    n = torch.randint(-40, 41, (T, 60), generator=torch.Generator().manual_seed(0)).double()
+    x = (n * step).to(DT[dtype]).to(gpu)
+    assert x.double().abs().max().item() == 40 * step and x[0].unique().numel() > 20
+    x[:, 7] = -0.0
+    check_topk(x, 8, grad=False)
+    check_topk(x, 8, groups=4, topk_groups=2, scoring="sigmoid", grad=False)
